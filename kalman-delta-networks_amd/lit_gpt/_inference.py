@@ -34,6 +34,47 @@ def clear_inference_caches(model: torch.nn.Module) -> None:
         m.__dict__.pop("_kdn_inference_cache", None)
 
 
+def parts_epoch(model: torch.nn.Module) -> int:
+    """How often parts of ``model`` have been exchanged by this package (``quantize_mx4``)."""
+    return model.__dict__.get("_kdn_parts_epoch", 0)
+
+
+def parts_exchanged(model: torch.nn.Module) -> None:
+    """Tell the decoders of ``model`` that a step captured before reads parts which it no longer has."""
+    model.__dict__["_kdn_parts_epoch"] = parts_epoch(model) + 1
+
+
+class StepSources:
+    """What a captured step of ``model`` reads beside its decoder's own buffers: every parameter and buffer, where the
+    model has it and its address and version, and the cached copies.  A graph replays on addresses, so what lies there
+    is kept from being released as long as this object is (a copy in the caches can be replaced by any later call)."""
+
+    def __init__(self, model: torch.nn.Module) -> None:
+        modules = list(model.modules())
+        self._parts = [(m._modules, n, c) for m in modules for n, c in m._modules.items()]
+        self._tensors = [(held, n, t, t.data_ptr(), t._version) for m in modules for held in (m._parameters, m._buffers)
+                         for n, t in held.items() if t is not None and not t.is_inference()]
+        # (an inference tensor has no version)
+        self._parts += [(held, n, t) for m in modules for held in (m._parameters, m._buffers)
+                        for n, t in held.items() if t is None or t.is_inference()]
+        self._copies = [dict(m.__dict__["_kdn_inference_cache"]) for m in modules if "_kdn_inference_cache" in m.__dict__]
+        self._epoch = parts_epoch(model)
+
+    def current(self) -> bool:
+        """The model still has these parts, parameters and buffers, and none was written since.  (0.15 ms at 18 layers.)"""
+        for held, n, part in self._parts:
+            if held.get(n) is not part:
+                return False
+        for held, n, t, at, version in self._tensors:
+            if held.get(n) is not t or t._version != version or t.data_ptr() != at:
+                return False
+        return True
+
+    def same_parts(self, model: torch.nn.Module) -> bool:
+        """The cheap part of ``current`` for every step: ``parts_exchanged`` has not been called."""
+        return self._epoch == parts_epoch(model)
+
+
 def _key(tensors):
     return tuple((t.data_ptr(), t._version, t.dtype, t.device) for t in tensors)
 
@@ -253,5 +294,5 @@ def decode_head(x, norm, head, model):
     return y.view(x.shape[0], 1, -1)
 
 
-__all__ = ("PACK_MAX_ROWS", "GEMV_MAX_ROWS", "use_packed", "clear_inference_caches", "packed_weight", "packed_bias",
-           "as_f32", "linear", "swiglu_gate", "decode_block", "decode_head")
+__all__ = ("PACK_MAX_ROWS", "GEMV_MAX_ROWS", "StepSources", "use_packed", "clear_inference_caches", "parts_epoch",
+           "parts_exchanged", "packed_weight", "packed_bias", "as_f32", "linear", "swiglu_gate", "decode_block", "decode_head")

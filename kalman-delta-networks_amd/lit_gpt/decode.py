@@ -11,11 +11,16 @@ about 20 otherwise), so at small batch the step is bound by launch overhead as m
 logits and every layer's state -- and each later step is one graph replay.  The decoder's layer
 states are in-place states (``KDNLayerState.inplace``): each layer advances its own buffers, the
 mixers through ``kdn_kalman_step`` (the single-token gain and memory update in one launch).
+
+A captured step reads the weights where they lay when it was captured.  The decoder keeps them, and the packed copies
+beside them, from being released; it captures again at the first step after ``quantize_mx4``, and after a ``prefill``
+that finds a parameter, buffer or part of the model exchanged or written since.
 """
 from __future__ import annotations
 
 import torch
 
+from ._inference import StepSources
 from .kdn_ops.sampling import sample_tokens
 from .kdn_state import KDNLayerState
 
@@ -27,6 +32,7 @@ class KDNDecoder:
         self.use_graph = bool(use_graph)
         self.state = None
         self.graph = None
+        self._sources = None
         dev = next(model.parameters()).device
         self.tokens = torch.zeros(self.B, 1, dtype=torch.long, device=dev)
         self.logits = None
@@ -37,6 +43,8 @@ class KDNDecoder:
         and keeps the state after it (copied into this decoder's fixed buffers)."""
         if idx.ndim != 2 or idx.shape[0] != self.B:
             raise ValueError(f"idx must have shape [{self.B}, T], got {tuple(idx.shape)}")
+        if self.graph is not None and not self._sources.current():
+            self._release()
         logits, state = self.model(idx, return_state=True)
         if self.state is None:
             self.state = [KDNLayerState(tuple(c.clone() for c in s.conv), s.memory.clone(), s.precision.clone(),
@@ -53,6 +61,11 @@ class KDNDecoder:
             s.precision.copy_(n.precision)
             for c, nc in zip(s.conv, n.conv):
                 c.copy_(nc)
+
+    def _release(self):
+        """Drop the captured step, and what was kept for it: replays may still be running on any stream."""
+        torch.cuda.synchronize(self.tokens.device)
+        self.graph = self._sources = None
 
     def _eager_step(self):
         # the states are in-place states: the layers advance their buffers themselves
@@ -76,9 +89,10 @@ class KDNDecoder:
             for c, sc in zip(s.conv, cs):
                 c.copy_(sc)
             s.seen_tokens = n
-        self.graph = torch.cuda.CUDAGraph()
-        with torch.cuda.graph(self.graph):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
             self._eager_step()
+        self.graph, self._sources = graph, StepSources(self.model)
         for s, (_, _, _, n) in zip(self.state, saved):
             s.seen_tokens = n  # capture records the step without running it
 
@@ -92,6 +106,8 @@ class KDNDecoder:
         if not self.use_graph:
             self._eager_step()  # advances seen_tokens itself
         else:
+            if self.graph is not None and not self._sources.same_parts(self.model):
+                self._release()
             if self.graph is None:
                 self._capture()
             self.graph.replay()

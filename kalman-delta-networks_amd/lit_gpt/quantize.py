@@ -13,7 +13,7 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from ._inference import clear_inference_caches
+from ._inference import clear_inference_caches, parts_exchanged
 from .kdn_ops.mx4 import MX4Tensor, mx4_linear, mx4_quantize
 from .model import GPT, LLaMAMLP, SwiGLU
 
@@ -70,10 +70,12 @@ def quantize_mx4(model: GPT, *, head: bool = True) -> GPT:
     """Replaces every block's SwiGLU and, with ``head``, the head by their MX4 forms, in place; returns ``model``.
 
     The weights must be on the GPU.  Activations must be bf16 (a bf16 model) and the model is for inference: its MX4
-    products refuse inputs that need a gradient.  The replaced weights are released, packed copies of them too."""
+    products refuse inputs that need a gradient.  The replaced weights are released, packed copies of them too (by a
+    ``KDNDecoder`` that has captured its step, at its next call, which captures it again)."""
     if not isinstance(model, GPT):
         raise TypeError(f"quantize_mx4 takes a GPT, got {type(model).__name__}")
     clear_inference_caches(model)
+    parts_exchanged(model)
     for block in model.transformer.h:
         mlp = getattr(block, "mlp", None)
         if type(mlp) is LLaMAMLP and type(mlp.swiglu) is SwiGLU:
