@@ -364,8 +364,8 @@ int kdn_mx4_dequantize(const void* codes, const void* scales, int64_t rows, int 
                        hipStream_t stream);
 /* y[m, n] = epilogue(sum_k x[m, k] W[n, k]), W [N, K] in MX4 (gated: [2N, K] = [W1; W2]), fp32 sums, bf16 out:
  * + bias; gated: silu(W1 x + b1) (W2 x + b2); + res[m, n]; one rounding.  x_scales NULL: x [M, K] bf16, K % 8 == 0,
- * rows x_row_stride elements apart (% 8 == 0), 16-byte aligned.  Otherwise x is MX4's codes (x_row_stride unused).
- * bias [N] ([2N] gated) and res [M, N] bf16 or NULL.  workspace: kdn_mx4_linear_workspace_size bytes, 16-byte
+ * rows x_row_stride elements apart (% 8 == 0, at most 2^21), 16-byte aligned.  Otherwise x is MX4's codes (x_row_stride
+ * unused).  bias [N] ([2N] gated) and res [M, N] bf16 or NULL.  workspace: kdn_mx4_linear_workspace_size bytes, 16-byte
  * aligned (0 bytes and NULL for M <= 16, and where K is not split).  K <= 2^20, N K < 2^34. */
 size_t kdn_mx4_linear_workspace_size(int M, int N, int K, int x_mx4, int gated);
 int kdn_mx4_linear(const void* x, const void* x_scales, int64_t x_row_stride, const void* W, const void* W_scales,

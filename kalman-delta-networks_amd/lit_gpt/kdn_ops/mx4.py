@@ -15,6 +15,7 @@ import torch
 from . import _lib
 
 GROUP = 128
+MAX_ROW_STRIDE = 1 << 21  # of bf16 x, in elements: kdn_mx4_linear addresses a tile's rows by 32-bit offsets
 
 
 class MX4Tensor(NamedTuple):
@@ -145,13 +146,14 @@ def mx4_linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optio
         res_stride = residual.stride(0)
     K8 = K
     if not quantized:
-        # the kernels load 16-byte pieces of rows: rows of another length or alignment are copied
+        # the kernels load 16-byte pieces of rows: rows of another length or alignment, or too far apart, are copied
         if K % 8:
             K8 = K + -K % 8
             padded = x2.new_zeros((M, K8))
             padded[:, :K] = x2
             x2 = padded
-        elif x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and (x2.stride(0) < K or x2.stride(0) % 8)):
+        elif x2.stride(1) != 1 or x2.data_ptr() % 16 or (M > 1 and (not K <= x2.stride(0) <= MAX_ROW_STRIDE
+                                                                    or x2.stride(0) % 8)):
             x2 = x2.clone(memory_format=torch.contiguous_format)
         row_stride = x2.stride(0)
     y = torch.empty((*lead, N), device=x2.device, dtype=torch.bfloat16)
