@@ -11,6 +11,7 @@ import os
 import pathlib
 
 import torch
+from torch.autograd import forward_ad
 
 _LIB_PATH = pathlib.Path(__file__).resolve().parent / "libkdn_hip.so"
 _lib = None
@@ -211,6 +212,18 @@ def is_bf16(t: torch.Tensor) -> int:
     if t.dtype == torch.float32:
         return 0
     raise TypeError(f"expected bf16 or fp32 tensor, got {t.dtype}")
+
+
+def refuse_derivatives(name: str, *tensors) -> None:
+    """An operator without derivatives refuses tensors that need a gradient or carry a tangent, rather than drop them."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise RuntimeError(f"{name} has no backward: call it under torch.no_grad()")
+    if getattr(forward_ad, "_current_level", 0) >= 0:  # (no level: nothing carries a tangent)
+        for t in tensors:
+            if t is not None and t.is_floating_point() and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError(f"{name} has no forward-mode derivative")
 
 
 def require_device(*tensors):

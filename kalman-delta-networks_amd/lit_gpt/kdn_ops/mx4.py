@@ -57,10 +57,6 @@ def _one_device(first: torch.Tensor, *others) -> None:
             _lib.require_device(first, *others)
 
 
-def _refuse_grad(name: str):
-    raise RuntimeError(f"{name} has no backward: call it under torch.no_grad()")
-
-
 def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
     """``x`` [..., K] (bf16 or fp32) in MX4, its leading dimensions as rows.
 
@@ -71,8 +67,7 @@ def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
         raise TypeError(f"x must be bf16 or fp32, got {x.dtype}")
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must have at least one column, got {tuple(x.shape)}")
-    if x.requires_grad and torch.is_grad_enabled():
-        _refuse_grad("mx4_quantize")
+    _lib.refuse_derivatives("mx4_quantize", x)
     _one_device(x)
     K = x.shape[-1]
     x2 = x if x.ndim == 2 else x.reshape(-1, K)
@@ -134,9 +129,7 @@ def mx4_linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optio
         raise ValueError(f"bias must be a contiguous bf16 [{R}] or None")
     if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != (*lead, N)):
         raise ValueError(f"residual must be bf16 {(*lead, N)}, got {residual.dtype} {tuple(residual.shape)}")
-    if torch.is_grad_enabled() and (x2.requires_grad or (bias is not None and bias.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
-        _refuse_grad("mx4_linear")
+    _lib.refuse_derivatives("mx4_linear", x2, bias, residual)
     _one_device(x2, x_scales, weight.codes, weight.scales, bias, residual)
     res_stride = 0
     if residual is not None:

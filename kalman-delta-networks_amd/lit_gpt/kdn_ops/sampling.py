@@ -55,7 +55,9 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor], *, temper
 
     Each setting is a number, or a tensor [rows] (fp32; ``top_k`` int32) with one for each row.  ``temperature`` 0 takes
     the largest logit (lowest index), with the log-probability at temperature 1; if it is 0 for the whole call ``noise``
-    may be None.  Tokens whose logit is -inf or NaN are never drawn; a row with no other gets token -1, logprob -inf."""
+    may be None.  Tokens whose logit is -inf or NaN are never drawn; a row with no other gets token -1, logprob -inf.
+
+    There is no derivative: inputs that require a gradient (while autograd is on) or carry a tangent are refused."""
     if logits.ndim != 2:
         raise ValueError(f"logits must be [rows, vocab], got {tuple(logits.shape)}")
     code = _DTYPES.get(logits.dtype)
@@ -73,6 +75,7 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor], *, temper
             raise ValueError("noise is needed unless temperature is 0")
     elif noise.shape != (B, V) or noise.dtype != torch.float32:
         raise ValueError(f"noise must be fp32 [{B}, {V}], got {noise.dtype} {tuple(noise.shape)}")
+    _lib.refuse_derivatives("sample_tokens", logits, noise, t_rows, p_rows, m_rows)
     dev = _lib.require_device(logits, noise, t_rows, k_rows, p_rows, m_rows)
     if (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
