@@ -25,13 +25,14 @@ def _hold(module: nn.Module, name: str, weight: torch.Tensor) -> None:
 
 
 class MX4Linear(nn.Module):
-    """``nn.Linear`` with an MX4 weight (bf16 activations, no backward)."""
+    """``nn.Linear`` with an MX4 weight (bf16 activations, no backward).  ``bias`` False leaves its bias out."""
 
-    def __init__(self, linear: nn.Linear) -> None:
+    def __init__(self, linear: nn.Linear, bias: bool = True) -> None:
         super().__init__()
         self.in_features, self.out_features = linear.in_features, linear.out_features
         _hold(self, "weight", linear.weight)
-        self.register_buffer("bias", None if linear.bias is None else linear.bias.detach().to(torch.bfloat16).clone())
+        keep = linear.bias if bias else None
+        self.register_buffer("bias", None if keep is None else keep.detach().to(torch.bfloat16).clone())
 
     @property
     def mx4(self) -> MX4Tensor:
@@ -81,7 +82,7 @@ def quantize_mx4(model: GPT, *, head: bool = True) -> GPT:
         if type(mlp) is LLaMAMLP and type(mlp.swiglu) is SwiGLU:
             mlp.swiglu = MX4SwiGLU(mlp.swiglu)
     if head and type(model.lm_head) is nn.Linear:
-        model.lm_head = MX4Linear(model.lm_head)
+        model.lm_head = MX4Linear(model.lm_head, bias=False)  # (``GPT.forward`` takes a linear head's weight alone)
     return model
 
 
