@@ -107,8 +107,9 @@ class GPT(nn.Module):
         logits = decode_head(x, self.transformer.ln_f, self.lm_head, self) if stateful else None
         if logits is None:
             x = self.transformer.ln_f(x)
-            # (a head of another type, as an MX4 one, has its own product)
-            logits = linear(x, self.lm_head.weight) if isinstance(self.lm_head, nn.Linear) else self.lm_head(x)
+            # of a head that has a weight the weight is used, whatever its type; an MX4 one has its own product
+            weight = getattr(self.lm_head, "weight", None)
+            logits = self.lm_head(x) if weight is None else linear(x, weight)
         return (logits, states) if return_state else logits
 
     @classmethod
