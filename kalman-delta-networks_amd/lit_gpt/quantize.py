@@ -10,6 +10,8 @@ The reference has no counterpart: its models run in bf16 and fp32.  The SwiGLU a
 """
 from __future__ import annotations
 
+import warnings
+
 import torch
 from torch import nn
 
@@ -66,23 +68,42 @@ class MX4SwiGLU(nn.Module):
         return mx4_linear(mx4_linear(x, self.w12, self.b12, gated=True), self.w3, self.b3, residual=residual)
 
 
+def _is_linear(module) -> bool:
+    """The call is the product with ``module.weight`` and the bias (a parametrised weight's value included)."""
+    return isinstance(module, nn.Linear) and type(module).forward is nn.Linear.forward and "forward" not in module.__dict__
+
+
+def _is_swiglu(module) -> bool:
+    return type(module) is SwiGLU and "forward" not in module.__dict__ and all(_is_linear(m) for m in (module.w1, module.w2, module.w3))
+
+
 @torch.no_grad()
 def quantize_mx4(model: GPT, *, head: bool = True) -> GPT:
     """Replaces every block's SwiGLU and, with ``head``, the head by their MX4 forms, in place; returns ``model``.
 
     The weights must be on the GPU.  Activations must be bf16 (a bf16 model) and the model is for inference: its MX4
     products refuse inputs that need a gradient.  The replaced weights are released, packed copies of them too (by a
-    ``KDNDecoder`` that has captured its step, at its next call, which captures it again)."""
+    ``KDNDecoder`` that has captured its step, at its next call, which captures it again), and hooks on the replaced
+    parts with them.  A part of another type, whose call may be more than its weights' products, stays as it is, with a
+    warning that names it."""
     if not isinstance(model, GPT):
         raise TypeError(f"quantize_mx4 takes a GPT, got {type(model).__name__}")
     clear_inference_caches(model)
     parts_exchanged(model)
-    for block in model.transformer.h:
+    kept = []
+    for i, block in enumerate(model.transformer.h):
         mlp = getattr(block, "mlp", None)
-        if type(mlp) is LLaMAMLP and type(mlp.swiglu) is SwiGLU:
-            mlp.swiglu = MX4SwiGLU(mlp.swiglu)
-    if head and type(model.lm_head) is nn.Linear:
+        swiglu = getattr(mlp, "swiglu", None)
+        if type(mlp) is LLaMAMLP and _is_swiglu(swiglu):
+            mlp.swiglu = MX4SwiGLU(swiglu)
+        elif mlp is not None and not (type(mlp) is LLaMAMLP and type(swiglu) is MX4SwiGLU):
+            kept.append(f"transformer.h.{i}.mlp")
+    if head and _is_linear(model.lm_head):
         model.lm_head = MX4Linear(model.lm_head, bias=False)  # (``GPT.forward`` takes a linear head's weight alone)
+    elif head and type(model.lm_head) is not MX4Linear:
+        kept.append("lm_head")
+    if kept:
+        warnings.warn(f"quantize_mx4 leaves parts of other types than the model's own as they are: {', '.join(kept)}", stacklevel=3)
     return model
 
 
