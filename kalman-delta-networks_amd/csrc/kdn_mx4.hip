@@ -137,8 +137,11 @@ __device__ __forceinline__ uint4 buf_ld16(bufrsrc r, uint32_t off) {
 constexpr uint32_t kOut = 0x80000000u;  // a buffer offset past every buffer: loads 0
 
 // silu(a) b; e^-a = inf for very negative a gives -0.  (The hardware's reciprocal and exponential, about 2^-22 off, before
-// a rounding to 8 bits: an IEEE division made the epilogue of 2304-element sums a quarter of the product's time.)
-__device__ __forceinline__ float mx_gate(float a, float b) { return a * frcp(1.f + fexp(-a)) * b; }
+// a rounding to 8 bits: an IEEE division made the epilogue of 2304-element sums a quarter of the product's time.)  The
+// reciprocal flushes subnormal results, so it is taken of a quarter of 1 + e^-a, at most 2^126 or infinite.
+__device__ __forceinline__ float mx_gate(float a, float b) {
+  return 0.25f * a * frcp(__builtin_fmaf(fexp(-a), 0.25f, 0.25f)) * b;
+}
 // One output of the epilogue, from the sum of W's row n (and, gated, of W2's).
 __device__ __forceinline__ float mx_epilogue(const MxArgs& A, int m, int n, float v0, float v1, bool gated) {
   float o = v0 + (A.bias ? bf2f(A.bias[n]) : 0.f);
