@@ -31,6 +31,15 @@ def _part(v):
     return 0 <= v <= 1
 
 
+# The kernel's scalars are fp32: a number past its range is taken as its nearest positive one (a temperature or top_p of
+# 1e-50 is not 0).
+_FP32 = torch.finfo(torch.float32)
+
+
+def _positive(v) -> float:
+    return 0.0 if v == 0 else min(max(float(v), _FP32.tiny), _FP32.max)
+
+
 def _setting(name: str, value, rows: int, dtype, ok, what: str):
     """(tensor or None, scalar) of a per-call or per-row setting."""
     if isinstance(value, torch.Tensor):
@@ -86,8 +95,8 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor], *, temper
     if B:
         with _lib.on(dev):
             _lib.call("kdn_sample", logits.data_ptr(), code, logits.stride(0), _lib.ptr(noise),
-                      0 if noise is None else noise.stride(0), _lib.ptr(t_rows), float(t), _lib.ptr(k_rows), min(k, V),
-                      _lib.ptr(p_rows), float(p), _lib.ptr(m_rows), float(m), B, V, tokens.data_ptr(),
+                      0 if noise is None else noise.stride(0), _lib.ptr(t_rows), _positive(t), _lib.ptr(k_rows), min(k, V),
+                      _lib.ptr(p_rows), _positive(p), _lib.ptr(m_rows), float(m), B, V, tokens.data_ptr(),
                       logprobs.data_ptr(), _lib.stream_of(logits))
     return tokens, logprobs
 
