@@ -133,7 +133,7 @@ def mx4_linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optio
     _one_device(x2, x_scales, weight.codes, weight.scales, bias, residual)
     res_stride = 0
     if residual is not None:
-        residual = residual if residual.ndim == 2 else residual.reshape(-1, N)
+        residual = residual if residual.ndim == 2 else residual.reshape(M, N)
         if (N > 1 and residual.stride(1) != 1) or (M > 1 and residual.stride(0) < N):
             residual = residual.contiguous()
         res_stride = residual.stride(0)
