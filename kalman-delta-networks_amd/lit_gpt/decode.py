@@ -117,26 +117,31 @@ class KDNDecoder:
 
     @torch.no_grad()
     def generate(self, idx: torch.Tensor, max_new_tokens: int, *, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
-                 generator=None):
+                 generator=None, vocab_size=None):
         """Runs the prompt ``idx`` [B,T] and draws ``max_new_tokens`` tokens after it, one per sequence and step, with
         ``sample_tokens`` (its settings: a number, or one per sequence); the random numbers come from ``generator``.
+        ``vocab_size``: only the first so many tokens can be drawn (the model's logits are as many as its
+        ``padded_vocab_size``, and no tokenizer has the padding's; the probabilities are those of the rest).
         Returns ``(tokens [B, max_new_tokens] int64, logprobs fp32)``.  A sequence without a token that can be drawn (its
         logits are all -inf or NaN) gets token -1, and goes on as if it were 0."""
         if max_new_tokens < 0:
             raise ValueError(f"max_new_tokens must be >= 0, got {max_new_tokens}")
         logits = self.prefill(idx)[:, -1]
+        V = logits.shape[1] if vocab_size is None else vocab_size
+        if not 1 <= V <= logits.shape[1]:
+            raise ValueError(f"vocab_size must be 1 to {logits.shape[1]}, got {vocab_size}")
         dev = logits.device
         tokens = torch.empty((self.B, max_new_tokens), device=dev, dtype=torch.int64)
         logprobs = torch.empty((self.B, max_new_tokens), device=dev, dtype=torch.float32)
         greedy = not isinstance(temperature, torch.Tensor) and temperature == 0
-        noise = None if greedy else torch.empty((self.B, logits.shape[1]), device=dev, dtype=torch.float32)
+        noise = None if greedy else torch.empty((self.B, V), device=dev, dtype=torch.float32)
         for i in range(max_new_tokens):
             if i:
                 logits = self.step(tokens[:, i - 1].clamp_min(0))  # (-1 is no row of the embedding)
             if noise is not None:
                 noise.exponential_(generator=generator)
-            tokens[:, i], logprobs[:, i] = sample_tokens(logits, noise, temperature=temperature, top_k=top_k, top_p=top_p,
-                                                         min_p=min_p)
+            tokens[:, i], logprobs[:, i] = sample_tokens(logits if vocab_size is None else logits[:, :V], noise,
+                                                         temperature=temperature, top_k=top_k, top_p=top_p, min_p=min_p)
         return tokens, logprobs
 
 
