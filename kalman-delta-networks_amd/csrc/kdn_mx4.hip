@@ -165,7 +165,7 @@ __device__ __forceinline__ uint32_t lds_address(const void* p) {
 __device__ __forceinline__ void dma16(u32x4 r, uint32_t lds, uint32_t voff, uint32_t soff) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, %3 offen lds" ::"s"(__builtin_amdgcn_readfirstlane(lds)),
                "v"(voff), "s"(r), "s"(__builtin_amdgcn_readfirstlane(soff))
-               : "memory");
+               : "m0", "memory");
 }
 __device__ __forceinline__ void dma_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
