@@ -239,3 +239,13 @@ def require_device(*tensors):
         elif t.device != dev:
             raise ValueError("all KDN tensors must share one device")
     return dev
+
+
+def one_device(first, *others) -> None:
+    """``require_device`` by the devices' numbers, for calls that are bound by the host."""
+    d = first.get_device()
+    if d < 0:
+        require_device(first)
+    for t in others:
+        if t is not None and t.get_device() != d:
+            require_device(first, *others)

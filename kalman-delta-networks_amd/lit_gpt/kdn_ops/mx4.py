@@ -48,15 +48,6 @@ def _check(name: str, t: MX4Tensor) -> int:
     return rows
 
 
-def _one_device(first: torch.Tensor, *others) -> None:
-    d = first.get_device()
-    if d < 0:
-        _lib.require_device(first)
-    for t in others:
-        if t is not None and t.get_device() != d:
-            _lib.require_device(first, *others)
-
-
 def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
     """``x`` [..., K] (bf16 or fp32) in MX4, its leading dimensions as rows.
 
@@ -68,7 +59,7 @@ def mx4_quantize(x: torch.Tensor) -> MX4Tensor:
     if x.ndim < 1 or x.shape[-1] < 1:
         raise ValueError(f"x must have at least one column, got {tuple(x.shape)}")
     _lib.refuse_derivatives("mx4_quantize", x)
-    _one_device(x)
+    _lib.one_device(x)
     K = x.shape[-1]
     x2 = x if x.ndim == 2 else x.reshape(-1, K)
     rows, groups = x2.shape[0], -(-K // GROUP)
@@ -89,7 +80,7 @@ def mx4_dequantize(t: MX4Tensor, dtype: torch.dtype = torch.float32) -> torch.Te
     rows = _check("t", t)
     if dtype != torch.bfloat16 and dtype != torch.float32:
         raise TypeError(f"dtype must be bf16 or fp32, got {dtype}")
-    _one_device(t.codes, t.scales)
+    _lib.one_device(t.codes, t.scales)
     y = torch.empty((rows, t.cols), device=t.codes.device, dtype=dtype)
     if rows:
         with _lib.on(y.device):
@@ -130,7 +121,7 @@ def mx4_linear(x: Union[torch.Tensor, MX4Tensor], weight: MX4Tensor, bias: Optio
     if residual is not None and (residual.dtype != torch.bfloat16 or residual.shape != (*lead, N)):
         raise ValueError(f"residual must be bf16 {(*lead, N)}, got {residual.dtype} {tuple(residual.shape)}")
     _lib.refuse_derivatives("mx4_linear", x2, bias, residual)
-    _one_device(x2, x_scales, weight.codes, weight.scales, bias, residual)
+    _lib.one_device(x2, x_scales, weight.codes, weight.scales, bias, residual)
     res_stride = 0
     if residual is not None:
         residual = residual if residual.ndim == 2 else residual.reshape(M, N)

@@ -33,11 +33,11 @@ def _part(v):
 
 # The kernel's scalars are fp32: a number past its range is taken as its nearest positive one (a temperature or top_p of
 # 1e-50 is not 0).
-_FP32 = torch.finfo(torch.float32)
+_TINY, _MAX = torch.finfo(torch.float32).tiny, torch.finfo(torch.float32).max
 
 
 def _positive(v) -> float:
-    return 0.0 if v == 0 else min(max(float(v), _FP32.tiny), _FP32.max)
+    return float(v) if _TINY <= v <= _MAX or v == 0 else _TINY if v < 1 else _MAX
 
 
 def _setting(name: str, value, rows: int, dtype, ok, what: str):
@@ -85,7 +85,8 @@ def sample_tokens(logits: torch.Tensor, noise: Optional[torch.Tensor], *, temper
     elif noise.shape != (B, V) or noise.dtype != torch.float32:
         raise ValueError(f"noise must be fp32 [{B}, {V}], got {noise.dtype} {tuple(noise.shape)}")
     _lib.refuse_derivatives("sample_tokens", logits, noise, t_rows, p_rows, m_rows)
-    dev = _lib.require_device(logits, noise, t_rows, k_rows, p_rows, m_rows)
+    _lib.one_device(logits, noise, t_rows, k_rows, p_rows, m_rows)
+    dev = logits.device
     if (V > 1 and logits.stride(1) != 1) or (B > 1 and logits.stride(0) < V):
         logits = logits.contiguous()
     if noise is not None and ((V > 1 and noise.stride(1) != 1) or (B > 1 and noise.stride(0) < V)):
