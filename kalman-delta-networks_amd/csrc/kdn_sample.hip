@@ -688,7 +688,16 @@ int launch_sample(SampleArgs A, int rows, hipStream_t stream) {
                                              hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
     if (e != hipSuccess) return (int)e;
   }
-  hipLaunchKernelGGL(sample_kernel<T>, dim3(rows), dim3(kThreads), lds, stream, A);
+  // a launch's threads are counted in 32 bits (of more rows the remainder alone would run)
+  constexpr int64_t kRows = 1 << 21;
+  for (int64_t r0 = 0; r0 < rows; r0 += kRows) {
+    SampleArgs P = A;
+    P.logits = static_cast<const T*>(A.logits) + r0 * A.ls, P.noise = A.noise ? A.noise + r0 * A.ns : nullptr;
+    P.tv = A.tv ? A.tv + r0 : nullptr, P.kv = A.kv ? A.kv + r0 : nullptr;
+    P.pv = A.pv ? A.pv + r0 : nullptr, P.mv = A.mv ? A.mv + r0 : nullptr;
+    P.tokens = A.tokens + r0, P.logprobs = A.logprobs + r0;
+    hipLaunchKernelGGL(sample_kernel<T>, dim3((unsigned)(rows - r0 < kRows ? rows - r0 : kRows)), dim3(kThreads), lds, stream, P);
+  }
   KDN_CHECK_LAUNCH();
   return 0;
 }
