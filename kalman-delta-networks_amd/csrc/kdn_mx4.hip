@@ -18,8 +18,8 @@ typedef int i32x8 __attribute__((ext_vector_type(8)));
 // Quantisation.  With E the exponent field of the block's largest magnitude, s = max(E - 2, 0) (so that magnitude
 // lies in [4, 8) units of 2^(s - 127)) and every element is rounded to the nearest of 0, 0.5, 1, 1.5, 2, 3, 4, 6
 // units, ties to the even code, larger ones to 6.  A block that holds an infinity or NaN gets s = 255.
-// A lane takes 8 elements, four lanes a block.  Bound by the bytes: 14416 x 2304 bf16 17.0 us (4.9 TB/s), back 13.5; 1999 x
-// 7208 fp32 11.4 and 14.3 (4.9 TB/s; with 8 fp32 a lane, every second 16 bytes to a store, 17.7).  A matrix whose rows
+// A lane takes 8 elements, four lanes a block.  Bound by the bytes: 14416 x 2304 bf16 17.1 us (4.9 TB/s), back 13.0; 1999 x
+// 7208 fp32 11.1 and 13.9 (4.7 TB/s; with 8 fp32 a lane, every second 16 bytes to a store, 17.7).  A matrix whose rows
 // start anywhere takes the same wide accesses (element by element, quantising and back 1999 x 7207 bf16 took 41 us, now 18).
 // ---------------------------------------------------------------------------------------------
 template <typename T>
@@ -187,8 +187,10 @@ __device__ __forceinline__ int turn(int row) {
 // bf16 x lies in LDS (loaded in the operand layout, four neighbouring lanes in four rows, M 8, K 7208 took 14000
 // accesses to L1 per workgroup); MX4 x, a quarter of that, in registers.  SW: groups per wave and chunk of K.  K past 8 SW
 // groups, or more of x than LDS holds, is walked in chunks of two buffers, x read again for every tile.
-// Gated N 7208, K 2304, M 1: 7.0 us (2.5 TB/s of W); N 2304, K 7208, M 8: 6.9 us.  Both are a few rounds of latency (launch,
-// W's first loads, the meeting in LDS), of which more loads in flight took nothing.
+// Gated N 7208, K 2304, M 1 to 8: 7.1 to 7.5 us (2.5 TB/s of W), M 16 8.7; N 2304, K 7208: M 1 5.4, M 4 5.7, M 8 6.7, M 16 (x
+// in four chunks) 11.7.  The waves spend half of the time in waits: a few rounds of latency (launch, W's first loads, the
+// meeting in LDS), of which more loads in flight took nothing, and at a long K from 8 rows on also x, all of which every
+// workgroup loads before its first product.
 constexpr int kFewWaves = 8, kFewLds = 131072;
 
 template <bool XQ, int NA, int SW>
@@ -366,9 +368,12 @@ int launch_few(const MxArgs& A, hipStream_t stream) {
 // With few tiles K is split over workgroups, whose fp32 sums a second kernel adds in order.
 // The outputs go through LDS to 16-byte stores at any alignment, the bias added to the sums once, the residual loaded 64 rows
 // ahead (3400 x 24423 of K 248 with both: 142 us; 2-byte accesses at their use 307).
-// M 4096, gated N 7208, K 2304: bf16 233 us (1.17 PFLOP/s, by the conversions of W to bf16 and the rounds of 912 tiles), MX4
-// 94 (2.9 PFLOP/s, by LDS).  M 64, N 32000, K 2304, bf16: 14.6 us (2.7 TB/s of W).  M 301, N 2304, K 7128, MX4: 13.5 us in 6
-// splits, and 4.2 for their sums.
+// M 4096, gated N 7208, K 2304: bf16 243 us (1.12 PFLOP/s), MX4 96 (2.8 PFLOP/s).  Neither fills a unit: the matrix cores
+// are busy for 49 % and 35 % of the time, LDS for 15 and 23, and the waves are in waits and barriers for 30 % and wait to
+// issue for 45 and 34: with two waves to a SIMD a stage's wait, reads, conversions and products run in turn; and 912 tiles
+// are 3.6 rounds.  (The clock goes by the inputs' values: of plain normal numbers the same products take 229 and 85 us.)
+// M 64, N 32000, K 2304, bf16: 15 us (2.6 TB/s of W; 41 % of the waves' time in waits, one workgroup to a CU and one stage
+// ahead).  M 301, N 2304, K 7128, MX4: 13.4 us in 4 splits, and 4.2 for their sums.
 constexpr int kGroupM = 4;  // tiles of x that run beside each other for every tile of W (an XCD's L2 holds both)
 
 template <bool XQ, int BM, int WM, int WN, int NT, int NA, int GS, bool SPLIT>

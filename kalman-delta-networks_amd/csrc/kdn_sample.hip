@@ -21,18 +21,20 @@
 // additions and a row's token is the same in every run (2^20 such masses fit 64 bits).
 //
 // One workgroup per row; the row is read from memory once, in 16-byte pieces that stay in LDS (of a longer row the rest
-// is read again from L2 by every pass).  Noise is read for the pieces that hold a kept token.  Bound by the vector
-// ALU of the row's CU (each operation on all of 32000 tokens is 500 cycles) and by the passes' barriers; with a row on every
-// CU the first pass and the draw also wait for HBM.  bf16, one row of 32000: top-k 50 and top-p 9.0 us, nothing 9.8, top-p
-// alone 15.8.  64 rows of 32000 with settings of their own 25 us, 256 rows of 50304 fp32 with top-p and min-p 38 us.
+// is read again from L2 by every pass).  Noise is read for the pieces that hold a kept token.  Bound by the passes
+// over the row on its one CU, one after the other (each operation on all of 32000 tokens is 500 cycles of its vector ALU): with
+// settings of their own 64 rows of 32000 take 26 us, in which the ALUs of their 64 CUs issue for 43 % of the time, the waves
+// spend 60 % in waits (barriers, LDS atomics, loads), and the other CUs are idle.  256 rows of 50304 fp32 with top-p and
+// min-p: 39 us, 41 % and 67 % (the first pass and the draw wait for HBM).  bf16, one row of 32000: top-k 50 and top-p 9.0 us,
+// nothing 9.6, top-p alone 16, greedy 7.3.
 #include "kdn_common.h"
 #include "../../include/kdn.h"
 
 namespace {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64, kBins = 2048, kList = 256;
-// Candidates are listed for k up to this: 64 rows of 32000 bf16 with top-p take 10.2 us for k 50, 13.4 for 150 and 16.1 for
-// 200 (by selection 20.9, 21.5 and 21.7); of k 250 there are more than the list holds, and 26.8 us.
+// Candidates are listed for k up to this: 64 rows of 32000 bf16 with top-p take 10.2 us for k 50, 13.6 for 150 and 16.1 for
+// 200 (by selection 20.9, 21.5 and 22.0); of k 250 there are more than the list holds, and 26.8 us (by selection 22.1).
 constexpr int kFew = 192;
 constexpr int kIdxBits = 20;
 constexpr float kMassOne = 1099511627776.f;  // 2^40
